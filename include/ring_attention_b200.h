@@ -366,7 +366,8 @@ int ra_cache4_read(const ra_cache4_t* cache, const ra_tensor_t* k, const ra_tens
  * weights_out (may be NULL) float32 [b, hkv, capacity]: cache->weights plus, for each row, the sum of
  * its probabilities over the lq queries and the heads that share it; it may be cache->weights itself.
  * Slots behind the last row are left as they are.  Results are the same bits at every call.
- * Channels of q are below 2^100 in magnitude (beyond, scores may leave the range of float32 on the way).
+ * Channels of q are below 2^100 in magnitude (beyond, scores may leave the range of float32 on the way), and so are those of
+ * the values (beyond, a key whose probability is 2^-20 or less of such a row's may be missing from the sum).
  * workspace: ra_cache4_attention_workspace bytes (negative: an argument error), 16-byte aligned, not
  * shared by calls that overlap; nothing in it is kept from call to call. */
 int64_t ra_cache4_attention_workspace(const ra_cache4_t* cache, int32_t h, int32_t lq, int32_t dtype);

@@ -574,9 +574,10 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<T, D, NT>) cache_attn_kern
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             x = fmaxf(x, m[nt][i]);
-            const float f = m[nt][i] == -INFINITY ? 0.f : ptx::ex2(m[nt][i] - x);
+            const float root = m[nt][i] == -INFINITY ? 0.f : ptx::ex2(0.5f * (m[nt][i] - x)), f = root * root;  // (part_root)
             m[nt][i] = x;
-            l[nt][i] *= f;
+            l[nt][i] *= root;
+            l[nt][i] *= root;
 #pragma unroll
             for (int c = 0; c < NG; ++c) {
               mid[nt][c][i] *= f;
@@ -763,8 +764,9 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<T, D, NT>) cache_attn_kern
         for (int x = 0; x < kWarps; ++x) top = fmaxf(top, jm[x * 8 + r]);
 #pragma unroll
         for (int x = 0; x < kWarps; ++x) {
-          f[x] = jm[x * 8 + r] == -INFINITY ? (jl[x * 8 + r] == jl[x * 8 + r] ? 0.f : NAN) : ptx::ex2(jm[x * 8 + r] - top);
-          total += f[x] * jl[x * 8 + r];
+          const float pl = jl[x * 8 + r], root = part_root(jm[x * 8 + r], pl, top);
+          f[x] = root * root;
+          total = fmaf(root, root * pl, total);
         }
         // cut at its start: this CTA's first part, else its second; a cluster's parts stay in its shared memory
         float* part = a.cluster ? jc + r * (D + 2) : a.part + (((int64_t)blockIdx.x * 2 + (w.first == 0)) * NT * 8 + nt * 8 + r) * kPartPitch<D>;
@@ -798,8 +800,8 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<T, D, NT>) cache_attn_kern
           for (int y = 0; y < a.cluster; ++y) top = fmaxf(top, cluster.map_shared_rank(jc, y)[r * (D + 2) + D]);
           for (int y = 0; y < a.cluster; ++y) {
             const float* part = cluster.map_shared_rank(jc, y) + r * (D + 2);
-            const float pm = part[D], pl = part[D + 1], f = pm == -INFINITY ? (pl == pl ? 0.f : NAN) : ptx::ex2(pm - top);
-            total = fmaf(f, pl, total);
+            const float pl = part[D + 1], root = part_root(part[D], pl, top), f = root * root;
+            total = fmaf(root, root * pl, total);
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) x[c] = fmaf(f, part[lane + 32 * c], x[c]);
           }
@@ -861,8 +863,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const __gri
     float y[V];
 #pragma unroll
     for (int j = 0; j < V; j += 2) *reinterpret_cast<float2*>(y + j) = *reinterpret_cast<const float2*>(src + 2 * lane + 32 * j);
-    const float f = m == -INFINITY ? (l == l ? 0.f : NAN) : ptx::ex2(m - top);
-    total = fmaf(f, l, total);
+    const float root = part_root(m, l, top), f = root * root;
+    total = fmaf(root, root * l, total);
 #pragma unroll
     for (int j = 0; j < V; ++j) x[j] = fmaf(f, y[j], x[j]);
   }

@@ -41,6 +41,9 @@ using namespace ptx;
 constexpr int kThreads = 288, kRows = kPromptRows, kKeys = kCacheUnit;
 constexpr float kLog2e = 1.4426950408889634f, kHeadroom = 6.f, kGrow = 8.f;
 constexpr int kLeastExp = -64, kMostExp = 126;
+// p 2^(f - m) of a unit whose f lies below this may be less than a float holds where larger values elsewhere set m, while p
+// itself still counts in the sum of probabilities, which is then formed without f.
+constexpr int kFarExp = -11;
 constexpr int kRoom = 2, kSpan = 10;  // a unit's exponents may lie this far below its common one, which starts kRoom above
 // The common exponent after a unit of largest exponent `most` that did not fit.
 __device__ __forceinline__ int next_common(int common, int most) {
@@ -449,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
         if (unit < 0) break;
         const int live = len - unit * kKeys, f_unit = side.f[0];
         const int4 odds = *reinterpret_cast<const int4*>(side.odd);
-        const bool odd = (odds.x | odds.y | odds.z | odds.w) != 0;
+        const bool odd = (odds.x | odds.y | odds.z | odds.w) != 0, apart = odd || f_unit < kFarExp;
         bool plain = !odd && live >= kKeys;
         if constexpr (MASKED) {
           const int lo = min(side.least_pos[0], side.least_pos[1]), hi = max(side.most_pos[0], side.most_pos[1]);
@@ -477,9 +480,9 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
         }
         const float peak = fmaf(max3(t[0], t[1], fmaxf(t[2], t[3])), scale, off - kHeadroom);
         if (__any_sync(0xffffffffu, peak > m + kGrow)) {
-          const float to = fmaxf(m, peak), by = m == -INFINITY ? 0.f : ex2(m - to);
+          const float to = fmaxf(m, peak), root = m == -INFINITY ? 0.f : ex2(0.5f * (m - to)), by = root * root;  // (part_root)
           m = to;
-          l *= by;
+          l = l * root * root;
           if (n > 0) {  // O is complete up to the unit before
             if (!(ok = WARP_WAIT(&sh.bars[O_DONE + (buf ^ 1)], (unit_phase >> (buf ^ 1) & 1) ^ 1))) break;
             tc_fence_after();
@@ -507,23 +510,23 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
           for (int j = 0; j < 16; ++j) {
             float x0, x1;
             unpack2(fma2(pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, a2), x0, x1);
+            r[2 * j] = __float_as_uint(x0), r[2 * j + 1] = __float_as_uint(x1);
             x0 = ex2(x0), x1 = ex2(x1);
             const __half2 h2 = __floats2half2_rn(x0, x1);
             pk[j] = *reinterpret_cast<const uint32_t*>(&h2);
             sum2 = add2(sum2, pack2(x0, x1));
-            r[2 * j] = __float_as_uint(x0), r[2 * j + 1] = __float_as_uint(x1);
           }
           tmem_st16(tmem_s + c * 16, pk);
-          if (!odd) {
+          if (!apart) {
             float s0, s1;
             unpack2(sum2, s0, s1);
             sum += s0 + s1;
-          } else {  // each key by its own power of two
+          } else {  // each key by its own power of two, which P may have taken below what a float holds
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum = fmaf(__uint_as_float(r[j]), two_to(f_unit - side.f[32 * c + j]), sum);
+            for (int j = 0; j < 32; ++j) sum += ex2(__uint_as_float(r[j]) - (float)side.f[32 * c + j]);
           }
         }
-        l = fmaf(sum, two_to(-f_unit), l);
+        l = fmaf(sum, apart ? 1.f : two_to(-f_unit), l);
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(&sh.bars[P_FULL + buf]);

@@ -9,6 +9,7 @@
 #include <climits>
 
 #include "cache4.cuh"
+#include "ptx_sm100.cuh"
 
 namespace ra {
 
@@ -38,6 +39,13 @@ constexpr int kMinUnits = 4;  // units of a run at least
 // Programmatic dependent launch: the kernel after this one may start its blocks / waits until the one before has ended.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// The root of the factor 2^(m - top) by which a part with reference m counts: 0 for one that saw nothing, NaN for one of NaN
+// alone (l is its sum).  The references follow the size of the values, so that the factor itself may be less than a float
+// holds where l, of smaller values, still counts; l is multiplied by the root twice.
+__device__ __forceinline__ float part_root(float m, float l, float top) {
+  return m == -INFINITY ? (l == l ? 0.f : NAN) : ptx::ex2(0.5f * (m - top));
+}
 
 // ---- schedule ----------------------------------------------------------------------------------------
 __device__ __forceinline__ int units_of(const CacheView& c, int b) {

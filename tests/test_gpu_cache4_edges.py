@@ -1,0 +1,81 @@
+"""Calls of the 4-bit key/value cache that its documentation allows and that lie at the edge of what its kernels divide up."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import ring_attention_b200 as ra
+from ring_attention_b200 import _lib
+from tests import cache4_oracle as O
+from tests.test_gpu_cache4 import BF16, F32, ROOM, Filled, _i32, _np, _rand
+
+pytestmark = pytest.mark.gpu
+
+
+def _filled(d, n, k, v, room=ROOM, dtype=BF16, positions=None):
+    """A cache of one sequence and head with the rows k, v [n, d] (NumPy), and the values that it stands for."""
+    cache = ra.KVCache4(1, 1, room or n, d)
+    k, v = (torch.from_numpy(np.asarray(x, np.float32)).cuda().to(dtype).view(1, n, 1, d) for x in (k, v))
+    cache.append(k, v, positions=None if positions is None else _i32(positions)[None])
+    return cache, O.values(_np(k)[0]), O.values(_np(v)[0])
+
+
+def _check_rows(q, k, v, kpos, qpos, out, lse, weights, scale, causal=False, form="many"):
+    """bf16 calls of one key/value head, with bounds that go by what each query sees and gives weight to.
+
+    A score is formed in fp32 from at most 3 * 16 partial products of a group's codes and its middle; with M the largest |k| of a
+    key's group it is off by at most e = 64 * 2^-24 scale sum |q| M + 4 * 2^-24 |s|.  The log-sum-exp is off by sum p e and 2^-21
+    and 2^-22 of itself; a probability by the factor 1 + e + that, the result by that of p |v|, by half a step of bf16 and, where
+    values are rounded to fp16, by 2^-12 of each and 2^-11 of each p; elsewhere by 2^-11 of p step code <= p (|v| + |min|)."""
+    lq, h, d = q.shape
+    n = len(k)
+    want = O.attend(q, k, v, np.asarray(kpos)[None], qpos, scale, causal=causal)
+    vis = np.asarray(kpos)[None] <= np.asarray(qpos)[:, None] if causal else np.ones((lq, n), bool)
+    group = np.abs(k[:, 0]).reshape(n, d // 64, 64).max(-1).repeat(64, 1)
+    least = np.abs(v[:, 0].reshape(n, d // 64, 64).min(-1)).repeat(64, 1)
+    size_v = np.abs(v[:, 0]) + (0 if form == "many" else least)
+    total, slack = np.zeros(n), np.zeros(n)
+    for i in range(h):
+        s = q[:, i] @ k[:, 0].T * scale
+        e = 64 * 2.0**-24 * (np.abs(q[:, i]) @ group.T) * scale + 4 * 2.0**-24 * np.abs(s)
+        p = np.where(vis, np.exp(np.where(vis, s, -np.inf) - want["lse"][i][:, None]), 0)
+        le = (p * e).sum(-1) + 2.0**-21 + 2.0**-22 * np.abs(want["lse"][i])
+        err = np.abs(_np(lse)[0, i] - want["lse"][i])
+        assert (err <= le).all(), (i, (err / le).max())
+        pe = p * (e + le[:, None])
+        tol = 2.0**-8 * np.abs(want["out"][:, i]) + 2 * pe @ np.abs(v[:, 0]) + (2.0**-10 * p) @ size_v
+        tol += 2.0**-24 * p.max() * np.abs(v[vis.any(0), 0]).max()
+        err = np.abs(_np(out)[0, :, i] - want["out"][:, i])
+        assert (err <= tol).all(), (i, (err / tol).max())
+        total += p.sum(0)
+        slack += 2 * pe.sum(0) + 2.0**-20 * p.sum(0)
+    w = _np(weights)[0, 0, :n]
+    assert (np.abs(w - total) <= slack + lq * h * 2.0**-125 + 2.0**-23 * total).all()
+
+
+# ---- many query rows: powers of two of the operands -------------------------------------------------------------
+@pytest.mark.parametrize("hidden", [True, False])
+@pytest.mark.parametrize("zero,loud", [((0, 1), 5), ((5, 6), 0), ((70, 71), 100), ((100, 101), 70), ((3, 4), 130), ((0, 64), 130), ((0, 100), 150),
+                                       ((64, 128), 5), ((1, 192), 0)])
+@pytest.mark.parametrize("size", [20, 64, 80, 100])
+@pytest.mark.parametrize("lq,room", [(70, ROOM), (2, None), (2, ROOM)])
+def test_rows_of_zeros_beside_rows_of_any_size(lq, room, size, zero, loud, hidden):
+    """Value rows of zeros and one of 2^size in a unit, or units apart; the large one in sight or behind a mask."""
+    rng = np.random.default_rng(size + zero[0])
+    d, n = 128, 192
+    k, v = rng.standard_normal((n, d)), rng.standard_normal((n, d)) + 0.3
+    v[zero[0]:zero[1]] = 0
+    v[loud] = np.ldexp(rng.standard_normal(d), size)
+    pos = np.arange(n)
+    pos[loud] = 5000 if hidden else pos[loud]
+    cache, kk, vv = _filled(d, n, k, v, room=room, positions=pos)
+    q = _rand(rng, (1, lq, 2, d), BF16)
+    q_pos = np.full(lq, n)
+    form = "many" if lq > 2 else "few"
+    for mod in (ra.ScoreMod(causal=True), None):
+        if mod is None and hidden:
+            continue
+        w = torch.zeros_like(cache.weights)
+        out, lse = ra.cache_attention(q, cache, q_positions=_i32(q_pos)[None], bias_fn=mod, return_lse=True, weights_out=w)
+        _check_rows(_np(q)[0], kk, vv, pos, q_pos, out, lse, w, d**-0.5, causal=mod is not None, form=form)
