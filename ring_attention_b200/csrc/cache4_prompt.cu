@@ -5,13 +5,16 @@
 // A CTA has 128 query rows and walks over units of 64 keys.  It decodes a unit's K and V once, into fp16 operands in
 // shared memory,   k' = step (code - 8) 2^-e   and   v' = (min + step code) 2^-f,
 // and then per unit:  S = Q K'^T + (group sums of q) (mid 2^-e)^T,  p = exp2(S 2^e factor + f - m),  O += P V'.
-// step has 8 significant bits and |code - 8| is at most 8, so k' is exact in fp16; the other part of a key, its groups'
-// mid = min + 8 step times the sums of q over the groups, is one more step of the product, of two-part factors (22 bits
-// each).  Scores, and L with them, so have fp32 accuracy as in the other form.  v' and P are rounded by 2^-12.
-// e and f are powers of two that bring the rows into fp16's range.  They are one number for a unit, a scalar in the
-// exponent, as long as the largest values of its rows are within 2^8 of one another; a unit where they are not, or that
-// holds NaN or infinities, gives each row its own and takes the form of the softmax that reads them per key, which is
-// also the form for masks and ALiBi.  m, the reference of the exponents, is the largest s + f less kHeadroom.
+// step has 8 significant bits and |code - 8| is at most 8, so k' is exact in fp16 where step 2^-e is 2^-17 or more (a group
+// whose step is less has one below 2^-26 of its row's largest value, or its row a power of two of its own: the loss is 2^-31
+// of that value at most); the other part of a key, its groups' mid = min + 8 step times the sums of q over the groups, is one
+// more step of the product, of two-part factors (22 bits each).  Scores, and L with them, so have fp32 accuracy as in the
+// other form.  v' and P are rounded by 2^-11 of themselves, values below 2^-19 of their row's largest by 2^-29 of that.
+// e and f are powers of two that bring the rows into fp16's range: largest values below 2^9 for K, where the two-part mids
+// are the limit, and 2^15 for V.  They are one number for a unit, a scalar in the exponent, as long as the largest values of
+// its rows are within 2^8 of one another; a unit where they are not, or that holds NaN or infinities, gives such rows their
+// own and takes the form of the softmax that reads them per key, which is also the form for masks and ALiBi.  m, the
+// reference of the exponents, is the largest s + f less kHeadroom.
 //
 // Warps 0 to 3 form the exponentials (a thread has a row of the tile, its lane of tensor memory), warps 4 to 7 decode (a
 // thread has a K or a V row of the unit), warp 8 issues the products.  Operands and S are double-buffered, so that the next
@@ -40,14 +43,17 @@ using namespace ptx;
 
 constexpr int kThreads = 288, kRows = kPromptRows, kKeys = kCacheUnit;
 constexpr float kLog2e = 1.4426950408889634f, kHeadroom = 6.f, kGrow = 8.f;
-constexpr int kLeastExp = -64, kMostExp = 126;
+// Exponents of rows: their largest value is below 2^(exponent + kTopK) or 2^(exponent + kTopV).
+constexpr int kTopK = 9, kTopV = 15;
+constexpr int kLeastExp = -64;  // of that value, and that of a row that is not there
+constexpr float kLeastStep = 0x1p-17f;  // of K, from which on its products with codes are exact
 // p 2^(f - m) of a unit whose f lies below this may be less than a float holds where larger values elsewhere set m, while p
 // itself still counts in the sum of probabilities, which is then formed without f.
-constexpr int kFarExp = -11;
+constexpr int kFarExp = -11 - kTopV;
 constexpr int kRoom = 2, kSpan = 10;  // a unit's exponents may lie this far below its common one, which starts kRoom above
 // The common exponent after a unit of largest exponent `most` that did not fit.
 __device__ __forceinline__ int next_common(int common, int most) {
-  return most > common || most < common - kSpan ? min(most + kRoom, kMostExp) : common;
+  return most > common || most < common - kSpan ? most + kRoom : common;
 }
 static_assert(kKeys == 64 && kRows == 128, "tile shapes are written out below");
 
@@ -133,24 +139,24 @@ __device__ __forceinline__ uint32_t two_parts(float x) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Exponent of the smallest power of two above x >= 0, within the range that the scaling takes.
-__device__ __forceinline__ int exponent_above(float x) {
-  return min(max((int)(__float_as_uint(x) >> 23) - 126, kLeastExp), kMostExp);
+// Exponent of a row of K or V whose largest value is x >= 0 (infinity, too: a sum of limits that is just beyond).
+__device__ __forceinline__ int row_exponent(float x, bool v) {
+  return max((int)(__float_as_uint(x) >> 23) - 126, kLeastExp) - (v ? kTopV : kTopK);
 }
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// Eight codes as fp16 values in the order 0 4 1 5 2 6 3 7:  K: step (code - 8), exact;  V: min + step code.  step16 is
-// step / 16, for codes in the upper half of a byte (0x6400 | x is 1024 + x, there 1024 + 16 code).
+// Eight codes as fp16 values in the order 0 4 1 5 2 6 3 7:  K: step (code - 8), exact;  V: min + step code.  0x6400 | code is
+// 1024 + code, and 0x5400 | 16 code, a code in the upper half of a byte, is 64 + code.
 template <bool V>
-__device__ __forceinline__ uint4 decode8(uint32_t w, __half2 step, __half2 step16, __half2 mn) {
+__device__ __forceinline__ uint4 decode8(uint32_t w, __half2 step, __half2 mn) {
   constexpr float base = V ? 0.f : 8.f;
-  const __half2 lo0 = __float2half2_rn(1024.f + base), hi0 = __float2half2_rn(1024.f + 16.f * base);
+  const __half2 lo0 = __float2half2_rn(1024.f + base), hi0 = __float2half2_rn(64.f + base);
   uint32_t r[4];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t lo = ((w >> (8 * i)) & 0x000f000fu) | 0x64006400u, hi = ((w >> (8 * i)) & 0x00f000f0u) | 0x64006400u;
+    const uint32_t lo = ((w >> (8 * i)) & 0x000f000fu) | 0x64006400u, hi = ((w >> (8 * i)) & 0x00f000f0u) | 0x54005400u;
     const __half2 a = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&lo), lo0), step, mn);
-    const __half2 b = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&hi), hi0), step16, mn);
+    const __half2 b = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&hi), hi0), step, mn);
     r[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
     r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
   }
@@ -201,7 +207,7 @@ struct KeyRow {
     using Sh = PromptShape<D>;
     const int row = thread & 63, warp = thread >> 5;
     const bool v = thread >= 64, there = row < live;
-    float step[NG], mn[NG];
+    float step[NG], mn[NG], least = INFINITY;  // smallest step that is not 0
     uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
@@ -210,9 +216,10 @@ struct KeyRow {
       const bool finite = fabsf(mn[i]) <= 3.4e38f && step[i] <= 3.4e38f;
       if (there && !finite) bad |= 1u << i;
       if (!there || !finite) step[i] = mn[i] = 0.f;  // (rows behind the last hold anything)
+      if (step[i] > 0.f) least = fminf(least, step[i]);
     }
-    const int own = there ? exponent_above(most()) : kLeastExp;
-    const bool fits = !there || (own <= common && own >= common - kSpan);
+    const int own = there ? row_exponent(most(), v) : kLeastExp - kTopV;
+    const bool fits = !there || (own <= common && own >= common - kSpan && (v || least * two_to(-common) >= kLeastStep));
     const int e = fits ? common : own;
     (v ? side.f : side.e)[row] = e;
     (v ? side.bad_v : side.bad_k)[row] = bad;
@@ -223,11 +230,10 @@ struct KeyRow {
       side.odd[warp] = odd;
     }
     const float scale = two_to(-e);
-    __half2 st[NG], s16[NG], off[NG];
+    __half2 st[NG], off[NG];
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       st[i] = __float2half2_rn(step[i] * scale);
-      s16[i] = __float2half2_rn(step[i] * scale * 0.0625f);
       off[i] = __float2half2_rn(v ? mn[i] * scale : 0.f);
     }
     char* const to = smem + (v ? Sh::kV : Sh::kK) + buf * NG * Sh::kKvPanel + row * 128;
@@ -244,7 +250,7 @@ struct KeyRow {
           const int n = 4 * i + j;
           const int c = kIsV ? n % NG : D == 64 ? 0 : 2 * (n >> 4) + ((n >> 1) & 1);
           const int chunk = kIsV ? n / NG : D == 64 ? n : 2 * ((n >> 2) & 3) + (n & 1);
-          *reinterpret_cast<uint4*>(to + c * Sh::kKvPanel + ((chunk ^ turn) << 4)) = decode8<kIsV>(w[j], st[c], s16[c], off[c]);
+          *reinterpret_cast<uint4*>(to + c * Sh::kKvPanel + ((chunk ^ turn) << 4)) = decode8<kIsV>(w[j], st[c], off[c]);
         }
       }
     };
@@ -602,12 +608,12 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
       if (unit >= 0) {
         raw.load(a.p.c, bh, unit, thread, MASKED);
         // the first unit's largest exponent is the one to go by
-        const int own = (thread & 63) < len - unit * kKeys ? exponent_above(raw.most()) : kLeastExp;
+        const int own = (thread & 63) < len - unit * kKeys ? row_exponent(raw.most(), thread >= 64) : kLeastExp - kTopV;
         const int largest = __reduce_max_sync(0xffffffffu, own);
         if (lane == 0) sh.first[warp - 4] = largest;
       }
       decoders_meet(true);
-      common = min(max(sh.first[(warp - 4) & 2], sh.first[(warp - 4) | 1]) + kRoom, kMostExp);
+      common = max(sh.first[(warp - 4) & 2], sh.first[(warp - 4) | 1]) + kRoom;
 
 #pragma unroll 1
       for (int i = 0;; ++i) {

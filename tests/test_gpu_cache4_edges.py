@@ -27,7 +27,7 @@ def _check_rows(q, k, v, kpos, qpos, out, lse, weights, scale, causal=False, for
     A score is formed in fp32 from at most 3 * 16 partial products of a group's codes and its middle; with M the largest |k| of a
     key's group it is off by at most e = 64 * 2^-24 scale sum |q| M + 4 * 2^-24 |s|.  The log-sum-exp is off by sum p e and 2^-21
     and 2^-22 of itself; a probability by the factor 1 + e + that, the result by that of p |v|, by half a step of bf16 and, where
-    values are rounded to fp16, by 2^-12 of each and 2^-11 of each p; elsewhere by 2^-11 of p step code <= p (|v| + |min|)."""
+    values are rounded to fp16, by 2^-11 of each and 2^-11 of each p; elsewhere by 2^-11 of p step code <= p (|v| + |min|)."""
     lq, h, d = q.shape
     n = len(k)
     want = O.attend(q, k, v, np.asarray(kpos)[None], qpos, scale, causal=causal)
@@ -79,3 +79,29 @@ def test_rows_of_zeros_beside_rows_of_any_size(lq, room, size, zero, loud, hidde
         w = torch.zeros_like(cache.weights)
         out, lse = ra.cache_attention(q, cache, q_positions=_i32(q_pos)[None], bias_fn=mod, return_lse=True, weights_out=w)
         _check_rows(_np(q)[0], kk, vv, pos, q_pos, out, lse, w, d**-0.5, causal=mod is not None, form=form)
+
+
+@pytest.mark.parametrize("hidden", [True, False])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("row,channel,group", [(1, 1, 1), (256, 1, 1), (64, 20, 1), (64, 50, 1), (1, 300, 1), (900, 1, 2.0**-4), (1, 1, 2.0**-12), (1, 1, 2.0**-24),
+                                               (900, 1000, 2.0**-9)])
+def test_rows_groups_and_channels_that_stand_out(d, row, channel, group, hidden):
+    """One row, one channel of all rows or all groups but the first of another size, in sight or behind a mask: the other keys' scores
+    and values are as near as ever.  Few keys have the weight, so that roundings do not cancel."""
+    rng = np.random.default_rng(int(row + channel))
+    n, lq = 320, 70
+    k, v = rng.standard_normal((n, d)) + 0.3, rng.standard_normal((n, d)) + 0.3
+    for x in (k, v):
+        x[:, 64:] *= group
+        x[:, 7] *= channel
+        x[70] *= row
+    pos = np.arange(n)
+    pos[70] = 5000 if hidden else 70
+    cache, kk, vv = _filled(d, n, k, v, positions=pos)
+    for scale in (d**-0.5, 1.0 / channel):
+        q = _rand(rng, (1, lq, 1, d), BF16)
+        q_pos = np.full(lq, n)
+        w = torch.zeros_like(cache.weights)
+        out, lse = ra.cache_attention(q, cache, q_positions=_i32(q_pos)[None], bias_fn=ra.ScoreMod(causal=True), return_lse=True, weights_out=w,
+                                      sm_scale=scale)
+        _check_rows(_np(q)[0], kk, vv, pos, q_pos, out, lse, w, scale, causal=True)
