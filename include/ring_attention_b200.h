@@ -322,7 +322,8 @@ int ra_ring_last_push(ra_ring_t* ring, int32_t backward, double* bytes, float* p
  * infinity or a value beyond the bf16 range reads back as NaN.  Codes lie in an order of the
  * library's own inside a row: fill, move and read rows through the calls below.
  *
- * All arrays are the caller's, on the device, contiguous and in the given shapes; a new cache
+ * All arrays are the caller's, on the device, contiguous and in the given shapes, the first five on
+ * 16-byte boundaries (k and v are read fastest on 32-byte ones); a new cache
  * has lengths and seen zeroed, the other arrays may hold anything.  The number of rows of a
  * sequence (lengths) and of the tokens it was ever given (seen) live on the device and are read
  * there, so calls captured into a graph stay right while the cache grows.  No call synchronises.

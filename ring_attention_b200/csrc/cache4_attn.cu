@@ -1340,6 +1340,7 @@ cudaError_t launch_cache_attn(const CacheAttnParams& p, cudaStream_t s) {
   a.vec_out = reinterpret_cast<uintptr_t>(p.out.ptr) % 16 == 0 && p.out.sb * es % 16 == 0 && p.out.sl * es % 16 == 0 && p.out.sh * es % 16 == 0;
   a.ctas = plan.ctas;
   a.vec = reinterpret_cast<uintptr_t>(p.q.ptr) % 16 == 0 && p.q.sb * es % 16 == 0 && p.q.sl * es % 16 == 0 && p.q.sh * es % 16 == 0;
+  a.wide = (reinterpret_cast<uintptr_t>(p.c.k) | reinterpret_cast<uintptr_t>(p.c.v)) % 32 == 0;
   char* ws = (char*)p.ws;
   a.part = (float*)(ws + plan.part);
   a.item = (int32_t*)(ws + plan.item);

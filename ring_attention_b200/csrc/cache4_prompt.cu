@@ -163,8 +163,14 @@ __device__ __forceinline__ uint4 decode8(uint32_t w, __half2 step, __half2 mn) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// 32 bytes at once: shared memory leaves next to no L1 cache, so that two halves of a sector would be fetched twice.
-__device__ __forceinline__ void load32(const void* p, uint4& lo, uint4& hi) {
+// 32 bytes at once: shared memory leaves next to no L1 cache, so that two halves of a sector would be fetched twice.  Arrays
+// that lie on 16-byte boundaries alone (`wide` false) are read that way all the same.
+__device__ __forceinline__ void load32(const uint4* p, bool wide, uint4& lo, uint4& hi) {
+  if (!wide) {
+    lo = p[0];
+    hi = p[1];
+    return;
+  }
   asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
                : "l"(p));
@@ -180,14 +186,15 @@ struct KeyRow {
   int pos;
 
   // `thread`: of the decoding warps, 0 to 127
-  __device__ __forceinline__ void load(const CacheView& c, int64_t bh, int unit, int thread, bool with_pos) {
+  __device__ __forceinline__ void load(const AttnArgs& a, int64_t bh, int unit, int thread, bool with_pos) {
+    const CacheView& c = a.p.c;
     const bool v = thread >= 64;
     const int slot = unit * kKeys + (thread & 63);
     const int64_t at = bh * c.cap + slot;
     const uint4* src = reinterpret_cast<const uint4*>(v ? c.v : c.k) + at * kVec;
     const int swap = v ? cache_v_swap(D, slot) : cache_k_swap(D, slot);  // (of whole 32 bytes)
 #pragma unroll
-    for (int i = 0; i < kVec; i += 2) load32(src + (i ^ swap), word[i], word[i + 1]);
+    for (int i = 0; i < kVec; i += 2) load32(src + (i ^ swap), a.wide, word[i], word[i + 1]);
 #pragma unroll
     for (int i = 0; i < NG; ++i) limits[i] = (v ? c.vl : c.kl)[at * NG + i];
     pos = with_pos && !v ? c.pos[at] : 0;
@@ -606,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
       int unit = sh.unit[0], next = sh.unit[1];
       int common = 0;
       if (unit >= 0) {
-        raw.load(a.p.c, bh, unit, thread, MASKED);
+        raw.load(a, bh, unit, thread, MASKED);
         // the first unit's largest exponent is the one to go by
         const int own = (thread & 63) < len - unit * kKeys ? row_exponent(raw.most(), thread >= 64) : kLeastExp - kTopV;
         const int largest = __reduce_max_sync(0xffffffffu, own);
@@ -625,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
           if (thread == 0) side.unit = unit;
           if (unit >= 0) {
             raw.decode(smem, buf, side, len - unit * kKeys, thread, common, MASKED);
-            if (next >= 0) raw.load(a.p.c, bh, next, thread, MASKED);
+            if (next >= 0) raw.load(a, bh, next, thread, MASKED);
           }
           fence_proxy_async_smem();
           mbar_arrive(&sh.bars[KV_FULL + buf]);

@@ -25,6 +25,7 @@ struct AttnArgs {
   int32_t ctas;      // CTAs launched
   int32_t vec;       // q rows on 16-byte boundaries
   int32_t vec_out;   // out rows on 16-byte boundaries
+  int32_t wide;      // k and v of the cache on 32-byte boundaries, and so all of their rows
   int32_t weights_group;  // units a CTA of the weights pass holds at a time
   float* part;       // [ctas][2][rows of a tile][kPartPitch]: unnormalised out, then max, then sum
   int32_t* item;     // [items][2]: first and last CTA

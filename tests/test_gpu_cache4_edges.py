@@ -105,3 +105,29 @@ def test_rows_groups_and_channels_that_stand_out(d, row, channel, group, hidden)
         out, lse = ra.cache_attention(q, cache, q_positions=_i32(q_pos)[None], bias_fn=ra.ScoreMod(causal=True), return_lse=True, weights_out=w,
                                       sm_scale=scale)
         _check_rows(_np(q)[0], kk, vv, pos, q_pos, out, lse, w, scale, causal=True)
+
+
+# ---- arrays of the caller's ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("d,lq", [(64, 70), (128, 70), (256, 70), (128, 2)])
+@pytest.mark.parametrize("off_k,off_v", [(16, 0), (0, 16), (48, 16)])
+def test_arrays_on_16_byte_boundaries(d, lq, off_k, off_v):
+    """Codes carved out of a pool: every call takes k and v that do not lie on 32-byte boundaries."""
+    f = Filled(d, [150, 64], 2, d, BF16, capacity=ROOM)
+    q = _rand(f.rng, (2, lq, 4, d), BF16)
+    mod = ra.ScoreMod(causal=True, window=90)
+    want = [ra.cache_attention(q, f.cache, bias_fn=m, return_lse=True) for m in (None, mod)]
+    there = [f.cache.read(150)]
+    nbytes = f.cache.k_codes.numel()
+    pool = torch.zeros(2 * nbytes + 256, dtype=torch.uint8, device="cuda")
+    assert pool.data_ptr() % 32 == 0 and nbytes % 32 == 0
+    k, v = pool[off_k:off_k + nbytes], pool[128 + nbytes + off_v:128 + 2 * nbytes + off_v]
+    k.copy_(f.cache.k_codes.flatten())
+    v.copy_(f.cache.v_codes.flatten())
+    f.cache._struct.k, f.cache._struct.v = k.data_ptr(), v.data_ptr()
+    got = [ra.cache_attention(q, f.cache, bias_fn=m, return_lse=True) for m in (None, mod)]
+    for x, y in zip(want + there, got + [f.cache.read(150)]):
+        for i in (0, 1):  # (the same rows see nothing)
+            assert torch.equal(torch.isnan(x[i]), torch.isnan(y[i])) and torch.equal(torch.nan_to_num(x[i]), torch.nan_to_num(y[i]))
+    f.cache.append(f.k[:, :1], f.v[:, :1])
+    f.cache.evict(100)
+    assert torch.isfinite(ra.cache_attention(q, f.cache)).all() and ra.device_status() == 0
