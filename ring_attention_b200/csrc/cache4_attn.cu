@@ -838,8 +838,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const __gri
   const int64_t bh = id / a.rows;
   const int row = (int)(id - bh * a.rows);
   const int64_t item = bh * a.tiles + row / tile_rows;
-  const int first = a.item[2 * item], splits = a.item[2 * item + 1] - first + 1;
-  if (splits <= 1) return;
+  const int first = a.item[2 * item], last = a.item[2 * item + 1];
+  if (!cache_note_holds(first, last, a.ctas)) return;  // (the status word tells; the whole block or warp has the one item)
+  const int splits = last - first + 1;
+  if (splits == 1) return;
   // the first CTA's second part, the others' first
   const float* part = a.part + ((int64_t)first * 2 * tile_rows + row % tile_rows) * kPartPitch<D>;
   const int64_t step = (int64_t)2 * tile_rows * kPartPitch<D>, second = (int64_t)tile_rows * kPartPitch<D>;

@@ -45,4 +45,8 @@ RA_HD int cache_v_swap(int d, int slot) { return cache_v_swizzle(d, slot) >> (d 
 // parity and rows 0, 2, 4, 6 in (bit 0, bit 2), which is what keeps the reads of K and V rows off one another's banks.
 RA_HD int cache_kappa(int r) { return r ^ ((r >> 1) & 1); }
 
+// Whether the note of an item's first and last CTA can be followed: a CTA whose wait ran out leaves items without one, and
+// the workspace there holds anything.
+RA_HD bool cache_note_holds(int first, int last, int ctas) { return first >= 0 && last >= first && last < ctas; }
+
 }  // namespace ra
