@@ -846,7 +846,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const __gri
   const float* part = a.part + ((int64_t)first * 2 * tile_rows + row % tile_rows) * kPartPitch<D>;
   const int64_t step = (int64_t)2 * tile_rows * kPartPitch<D>, second = (int64_t)tile_rows * kPartPitch<D>;
   auto part_of = [&](int i) { return part + (i ? i * step : second); };
-  __shared__ float s_top[kJoinWarps], s_sum[kJoinWarps], s_out[SOLO ? 1 : kJoinWarps][D];
+  __shared__ float s_top[kJoinWarps], s_sum[kJoinWarps];
+  __shared__ __align__(16) float s_out[SOLO ? 1 : kJoinWarps][D];  // (written in pairs)
   float top = -INFINITY;
   for (int i = SOLO ? lane : threadIdx.x; i < splits; i += kStep * 32) top = fmaxf(top, part_of(i)[D]);
 #pragma unroll
