@@ -348,7 +348,8 @@ typedef struct ra_cache4 {
 /* Adds rows: k, v [b, t, hkv, d] of `dtype`, the first counts[i] of sequence i (NULL: all t) at the
  * slots from start[i] on (NULL: behind the last; else clipped to 0..lengths[i], and what lies behind
  * the new rows is dropped: the way back from rejected draft tokens).  positions [b, t] (NULL: go on
- * where the sequence stands, less the rows dropped).  New rows have weight 0.  Then lengths = start +
+ * where the sequence stands; where rows are dropped, at the position of the first of them, or behind the
+ * row before it where that is later).  New rows have weight 0.  Then lengths = start +
  * count and seen = position of the last row + 1.  Rows beyond the capacity are dropped and bit 17 of
  * the device status word is set. */
 int ra_cache4_append(const ra_cache4_t* cache, const ra_tensor_t* k, const ra_tensor_t* v, int32_t dtype, int32_t t,

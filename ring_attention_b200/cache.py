@@ -116,7 +116,8 @@ class KVCache4:
 
         `counts` [b]: only the first counts[i] rows of sequence i (a padded batch).  `start` [b]: from slot
         start[i] on instead of behind the last row, dropping what lies behind the new rows (rejected drafts).
-        `positions` [b, t]: default is to go on where the sequence stands.  Rows beyond the capacity are
+        `positions` [b, t]: default is to go on where the sequence stands, with `start` at the position of the first
+        row dropped, or behind the row before it where that is later (branches of drafts repeat positions).  Rows beyond the capacity are
         dropped and set bit 17 of `device_status()`."""
         shape = (self.batch, k.shape[1] if k.dim() == 4 else -1, self.kv_heads, self.head_dim)
         if k.shape != shape or v.shape != shape:

@@ -230,7 +230,14 @@ __device__ __forceinline__ AppendSpan append_span(const AppendParams& p, int b) 
   AppendSpan s;
   s.at = p.start ? min(max(p.start[b], 0), len) : len;
   s.count = p.counts ? min(max(p.counts[b], 0), p.t) : p.t;
-  s.pos = p.c.seen[b] - (len - s.at);
+  s.pos = p.c.seen[b];
+  if (s.at < len) {
+    // The first row that is dropped had the position to go on from, unless the row before it went further (branches of drafts:
+    // 10, 11, 11, of which two stay).  Rows that eviction has moved lie earlier, and all heads hold the same last rows.
+    const int32_t* pos = p.c.pos + (int64_t)b * p.c.hkv * p.c.cap;
+    s.pos = pos[s.at];
+    if (s.at > 0) s.pos = max(s.pos, pos[s.at - 1] + 1);
+  }
   return s;
 }
 // The counters after the rows are there: one thread a sequence.
@@ -305,6 +312,16 @@ __global__ void __launch_bounds__(kRowThreads, 4) cache_append_kernel(AppendPara
 __global__ void cache_counters_kernel(AppendParams p) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b < p.c.b) append_counters(p, b, append_span(p, b));
+}
+
+// Drops the rows from start on, ahead of an append by several blocks a sequence: they overwrite the positions that say where
+// to go on.
+__global__ void cache_drop_kernel(AppendParams p) {
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b >= p.c.b) return;
+  const AppendSpan s = append_span(p, b);
+  p.c.len[b] = s.at;
+  p.c.seen[b] = s.pos;
 }
 
 // ---- read --------------------------------------------------------------------------------------------
@@ -577,9 +594,14 @@ cudaError_t launch_cache_append(const CacheView& c, TensorView k, TensorView v, 
   p.status = device_status_word();
   if (!p.status) return cudaErrorInvalidSymbol;
   // One launch where one block a sequence does all its rows (a token each, or a few), else the counters that the
-  // blocks of a sequence all read are brought up to date by a launch of their own.
+  // blocks of a sequence all read are brought up to date by a launch of their own, and so are rows dropped before.
   const int tiles = (t + kRowTile - 1) / kRowTile;
   const bool one = tiles == 1;
+  if (start && !one) {
+    cache_drop_kernel<<<(c.b + 127) / 128, 128, 0, s>>>(p);
+    count_launch();
+    p.start = nullptr;
+  }
   cudaError_t e = by_type_and_dim(dtype, c.d, [&](auto tag, auto dim) {
     cache_append_kernel<decltype(tag), decltype(dim)::value><<<(unsigned)c.b * tiles, kRowThreads, 0, s>>>(p, tiles, one);
   });

@@ -131,3 +131,64 @@ def test_arrays_on_16_byte_boundaries(d, lq, off_k, off_v):
     f.cache.append(f.k[:, :1], f.v[:, :1])
     f.cache.evict(100)
     assert torch.isfinite(ra.cache_attention(q, f.cache)).all() and ra.device_status() == 0
+
+
+# ---- rows taken back -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", [1, 5, 40])
+@pytest.mark.parametrize("evicted", [False, True])
+def test_positions_after_drafts_that_branch(t, evicted):
+    """Drafts of one tree repeat positions; what is appended in their place goes on behind the rows that stay."""
+    rng = np.random.default_rng(t)
+    b, hkv, d, n = 4, 2, 64, 30
+    cache = ra.KVCache4(b, hkv, 200, d)
+    rows = lambda x: [_rand(rng, (b, x, hkv, d), BF16) for _ in range(2)]  # noqa: E731
+    cache.append(*rows(n))
+    at = n
+    if evicted:  # slots are no positions from here on, and the last rows may be gone
+        cache.weights.copy_(torch.rand_like(cache.weights))
+        cache.evict(20)
+        at = 20
+    assert cache.seen.tolist() == [n] * b
+    # at `n` one branch and its sibling, then the branch's child: positions n, n + 1, n + 1, n + 2
+    cache.append(*rows(4), positions=_i32([[n, n + 1, n + 1, n + 2]] * b))
+    assert cache.seen.tolist() == [n + 3] * b and cache.lengths.tolist() == [at + 4] * b
+    keep = [0, 1, 2, 4]  # drafts that stay: none, the first, the branch, all
+    then = [n, n + 1, n + 2, n + 3]
+    cache.append(*rows(t), start=_i32([at + x for x in keep]))
+    assert cache.lengths.tolist() == [at + x + t for x in keep]
+    assert cache.seen.tolist() == [x + t for x in then]
+    for i in range(b):
+        for j in range(hkv):
+            assert cache.positions[i, j, at + keep[i]:at + keep[i] + t].tolist() == list(range(then[i], then[i] + t))
+    # no rows in their place: the sequence stands where it stood before the last ones
+    cache.append(*rows(t), start=_i32([at + x for x in keep]), counts=_i32([0] * b))
+    assert cache.lengths.tolist() == [at + x for x in keep] and cache.seen.tolist() == then
+    q = _rand(rng, (b, 1, hkv, d), BF16)
+    one = ra.cache_attention(q, cache, bias_fn=ra.ScoreMod(causal=True, window=7))
+    want = ra.cache_attention(q, cache, q_positions=_i32([[x - 1] for x in then]), bias_fn=ra.ScoreMod(causal=True, window=7))
+    assert torch.equal(torch.nan_to_num(one), torch.nan_to_num(want)) and ra.device_status() == 0
+
+
+def test_start_in_a_graph_with_more_rows_than_a_block_takes():
+    """Replays of a captured append that drops rows: the counters and positions that a replay finds are those of the one before."""
+    rng = np.random.default_rng(3)
+    cache = ra.KVCache4(2, 1, 200, 64)
+    k, v = (_rand(rng, (2, 40, 1, 64), BF16) for _ in range(2))
+    start = _i32([10, 0])
+    cache.append(k, v)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.append(k, v, start=start)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.append(k, v, start=start)
+    for at in ([3, 40], [0, 45], [40, 99]):
+        start.copy_(_i32(at))
+        before = cache.lengths.tolist()
+        graph.replay()
+        at = [min(x, n) for x, n in zip(at, before)]
+        assert cache.lengths.tolist() == [x + 40 for x in at] == cache.seen.tolist()
+        for i in range(2):
+            assert cache.positions[i, 0, :at[i] + 40].tolist() == list(range(at[i] + 40))
