@@ -134,7 +134,11 @@ class KVCache4:
         positions = self._per_sequence("positions", positions, (self.batch, t))
         dtype = _dtype_code(k)
         if t == 0:
-            return
+            if start is None:
+                return
+            # nothing comes in the dropped rows' place: a row for each sequence of which none counts
+            k = v = k.new_zeros((self.batch, 1, self.kv_heads, self.head_dim))
+            t, positions, counts = 1, None, torch.zeros_like(start)
         k, v = _blhd(k.detach()), _blhd(v.detach())
         with _On(self.device) as stream:
             check(lib.ra_cache4_append(self._ref, _view(k), _view(v), dtype, t, _ptr(counts),

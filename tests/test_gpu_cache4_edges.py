@@ -192,3 +192,20 @@ def test_start_in_a_graph_with_more_rows_than_a_block_takes():
         assert cache.lengths.tolist() == [x + 40 for x in at] == cache.seen.tolist()
         for i in range(2):
             assert cache.positions[i, 0, :at[i] + 40].tolist() == list(range(at[i] + 40))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_no_rows_at_start_drop_what_is_behind(dtype):
+    rng = np.random.default_rng(5)
+    cache = ra.KVCache4(3, 2, 100, 128)
+    k, v = _rand(rng, (3, 30, 2, 128), dtype), _rand(rng, (3, 30, 2, 128), dtype)
+    cache.append(k, v)
+    was = cache.read(30)
+    cache.append(k[:, :0], v[:, :0])  # nothing to add, nothing to drop
+    assert cache.lengths.tolist() == [30] * 3
+    cache.append(k[:, :0], v[:, :0], start=_i32([7, 0, 99]))
+    assert cache.lengths.tolist() == [7, 0, 30] == cache.seen.tolist()
+    for x, y in zip(was, cache.read(30)):
+        assert torch.equal(x[0, :7], y[0, :7]) and torch.equal(x[2], y[2]) and y[0, 7:].abs().max() == 0
+    cache.append(k[:, :1], v[:, :1])
+    assert cache.positions[:, 1, :].gather(1, cache.lengths[:, None].long() - 1).flatten().tolist() == [7, 0, 30]
