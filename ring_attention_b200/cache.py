@@ -118,7 +118,7 @@ class KVCache4:
         start[i] on instead of behind the last row, dropping what lies behind the new rows (rejected drafts).
         `positions` [b, t]: default is to go on where the sequence stands, with `start` at the position of the first
         row dropped, or behind the row before it where that is later (branches of drafts repeat positions).  Rows beyond the capacity are
-        dropped and set bit 17 of `device_status()`."""
+        dropped and set bit 17 of `device_status()`.  There is no backward pass: the cache holds rounded copies."""
         shape = (self.batch, k.shape[1] if k.dim() == 4 else -1, self.kv_heads, self.head_dim)
         if k.shape != shape or v.shape != shape:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [{self.batch}, t, {self.kv_heads}, {self.head_dim}]")
@@ -129,6 +129,8 @@ class KVCache4:
         t = shape[1]
         if t > self.capacity:
             raise ValueError(f"{t} rows do not fit a capacity of {self.capacity}")
+        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+            raise _lib.RingAttentionError("KVCache4.append has no backward pass: call it under torch.no_grad() or detach k and v")
         counts = self._per_sequence("counts", counts, (self.batch,))
         start = self._per_sequence("start", start, (self.batch,))
         positions = self._per_sequence("positions", positions, (self.batch, t))
@@ -139,7 +141,7 @@ class KVCache4:
             # nothing comes in the dropped rows' place: a row for each sequence of which none counts
             k = v = k.new_zeros((self.batch, 1, self.kv_heads, self.head_dim))
             t, positions, counts = 1, None, torch.zeros_like(start)
-        k, v = _blhd(k.detach()), _blhd(v.detach())
+        k, v = _blhd(k), _blhd(v)
         with _On(self.device) as stream:
             check(lib.ra_cache4_append(self._ref, _view(k), _view(v), dtype, t, _ptr(counts),
                                        _ptr(start), _ptr(positions), stream))

@@ -209,3 +209,18 @@ def test_no_rows_at_start_drop_what_is_behind(dtype):
         assert torch.equal(x[0, :7], y[0, :7]) and torch.equal(x[2], y[2]) and y[0, 7:].abs().max() == 0
     cache.append(k[:, :1], v[:, :1])
     assert cache.positions[:, 1, :].gather(1, cache.lengths[:, None].long() - 1).flatten().tolist() == [7, 0, 30]
+
+
+# ---- refusals --------------------------------------------------------------------------------------------------
+def test_append_refuses_what_asks_for_a_gradient():
+    cache = ra.KVCache4(1, 1, 64, 64)
+    x = torch.ones(1, 2, 1, 64, device="cuda")
+    y = x.clone().requires_grad_(True)
+    for k, v in ((y, x), (x, y), (y * 2, x)):
+        with pytest.raises(ra.RingAttentionError):
+            cache.append(k, v)
+    assert cache.lengths.tolist() == [0]
+    with torch.no_grad():
+        cache.append(y, y)
+    cache.append(y.detach(), x)
+    assert cache.lengths.tolist() == [4]
