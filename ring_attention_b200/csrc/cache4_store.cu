@@ -222,9 +222,21 @@ struct AppendParams {
   unsigned int* status;
 };
 
+// Accesses to a position that several blocks may make at once.
+__device__ __forceinline__ int load_relaxed(const int32_t* p) {
+  int x;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(x) : "l"(p) : "memory");
+  return x;
+}
+__device__ __forceinline__ void store_relaxed(int32_t* p, int x) { asm volatile("st.relaxed.gpu.global.s32 [%0], %1;" ::"l"(p), "r"(x) : "memory"); }
+
 struct AppendSpan {
   int at, count, pos;  // first slot, rows, default position of the first row
 };
+// Where rows are dropped, the first of them had the position to go on from, unless the row before it went further (branches of
+// drafts: 10, 11, 11, of which two stay).  Rows that eviction has moved lie earlier, and all heads hold the same last rows.
+// Another block, or the counters below, may find the position in place of the dropped row's that is formed here, which gives
+// the same again.  (Or one of the caller's; then this one stands for no row and no counter.)
 __device__ __forceinline__ AppendSpan append_span(const AppendParams& p, int b) {
   const int len = min(max(p.c.len[b], 0), p.c.cap);
   AppendSpan s;
@@ -232,11 +244,9 @@ __device__ __forceinline__ AppendSpan append_span(const AppendParams& p, int b) 
   s.count = p.counts ? min(max(p.counts[b], 0), p.t) : p.t;
   s.pos = p.c.seen[b];
   if (s.at < len) {
-    // The first row that is dropped had the position to go on from, unless the row before it went further (branches of drafts:
-    // 10, 11, 11, of which two stay).  Rows that eviction has moved lie earlier, and all heads hold the same last rows.
     const int32_t* pos = p.c.pos + (int64_t)b * p.c.hkv * p.c.cap;
-    s.pos = pos[s.at];
-    if (s.at > 0) s.pos = max(s.pos, pos[s.at - 1] + 1);
+    s.pos = load_relaxed(pos + s.at);
+    if (s.at > 0) s.pos = max(s.pos, load_relaxed(pos + s.at - 1) + 1);
   }
   return s;
 }
@@ -302,7 +312,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) cache_append_kernel(AppendPara
       kdst[(int64_t)slot * (D / 8) + cache_k_word(D, c, e, slot)] = xw;
       vdst[(int64_t)slot * (D / 8) + cache_v_word(D, c, e, slot)] = yw;
       if (e < 2) ldst[(int64_t)slot * NG] = e ? yl : xl;
-      else if (c == 0 && e == 2) p.c.pos[head + slot] = p.positions ? p.positions[(int64_t)b * p.t + row0 + row] : s.pos + row0 + row;
+      else if (c == 0 && e == 2) store_relaxed(p.c.pos + head + slot, p.positions ? p.positions[(int64_t)b * p.t + row0 + row] : s.pos + row0 + row);
       else if (c == 0 && e == 3) p.c.weight[head + slot] = 0.f;
     }
   }
@@ -312,16 +322,6 @@ __global__ void __launch_bounds__(kRowThreads, 4) cache_append_kernel(AppendPara
 __global__ void cache_counters_kernel(AppendParams p) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b < p.c.b) append_counters(p, b, append_span(p, b));
-}
-
-// Drops the rows from start on, ahead of an append by several blocks a sequence: they overwrite the positions that say where
-// to go on.
-__global__ void cache_drop_kernel(AppendParams p) {
-  const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  if (b >= p.c.b) return;
-  const AppendSpan s = append_span(p, b);
-  p.c.len[b] = s.at;
-  p.c.seen[b] = s.pos;
 }
 
 // ---- read --------------------------------------------------------------------------------------------
@@ -594,14 +594,9 @@ cudaError_t launch_cache_append(const CacheView& c, TensorView k, TensorView v, 
   p.status = device_status_word();
   if (!p.status) return cudaErrorInvalidSymbol;
   // One launch where one block a sequence does all its rows (a token each, or a few), else the counters that the
-  // blocks of a sequence all read are brought up to date by a launch of their own, and so are rows dropped before.
+  // blocks of a sequence all read are brought up to date by a launch of their own.
   const int tiles = (t + kRowTile - 1) / kRowTile;
   const bool one = tiles == 1;
-  if (start && !one) {
-    cache_drop_kernel<<<(c.b + 127) / 128, 128, 0, s>>>(p);
-    count_launch();
-    p.start = nullptr;
-  }
   cudaError_t e = by_type_and_dim(dtype, c.d, [&](auto tag, auto dim) {
     cache_append_kernel<decltype(tag), decltype(dim)::value><<<(unsigned)c.b * tiles, kRowThreads, 0, s>>>(p, tiles, one);
   });
