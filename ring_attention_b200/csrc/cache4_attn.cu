@@ -586,6 +586,34 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm<T, D, NT>) cache_attn_kern
             }
           }
       }
+      if constexpr (MASKED) {
+        // A group of V that is NaN has to reach every row that sees its key, and below p = 0 stands for a key that is hidden: p of
+        // such keys stays above 0.
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int c = 0; c < NG; ++c) sum += limit_step(vlim[u][half][c]);
+        if (__any_sync(0xffffffffu, sum != sum)) {
+#pragma unroll
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float key = 0.f;
+#pragma unroll
+              for (int c = 0; c < NG; ++c) key += limit_step(vlim[u][half][c]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  float& x = s[u][nt][2 * half + i];
+                  if (key != key && x > -INFINITY) x = fmaxf(x, m[nt][i] - 120.f);
+                }
+            }
+        }
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -211,6 +211,31 @@ def test_no_rows_at_start_drop_what_is_behind(dtype):
     assert cache.positions[:, 1, :].gather(1, cache.lengths[:, None].long() - 1).flatten().tolist() == [7, 0, 30]
 
 
+# ---- NaN under masks -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,lq,room", [(F32, 2, None), (F32, 2, ROOM), (BF16, 2, None), (BF16, 2, ROOM), (BF16, 40, None), (BF16, 70, ROOM)])
+@pytest.mark.parametrize("at", [0, 130, 199])
+def test_nan_reaches_rows_that_see_it_however_little_they_weigh_it(dtype, lq, room, at):
+    """ALiBi takes the probability of a key far behind the query below what a float holds; its NaN value counts all the same, and
+    a key outside the window or behind the query does not."""
+    f = Filled(31, [200], 2, 128, dtype, capacity=room)
+    v = f.v.clone()
+    v[0, at, 1, 70] = float("nan")
+    f.cache.append(f.k, v, start=_i32([0]))
+    q = _rand(f.rng, (1, lq, 4, 128), dtype)
+    slopes = torch.tensor([0.0, 40.0, 0.0, 40.0], device="cuda")
+    for window in (0, 150):
+        pos = torch.arange(100, 100 + 3 * lq, 3, device="cuda")[None]
+        mod = ra.ScoreMod(causal=True, alibi_slopes=slopes, window=window)
+        out, lse = ra.cache_attention(q, f.cache, q_positions=pos, bias_fn=mod, return_lse=True)
+        sees = (pos[0] >= at) & ((pos[0] - at < window) if window else True)
+        for h in range(4):
+            bad = torch.zeros(lq, 128, dtype=torch.bool, device="cuda")
+            if h >= 2:
+                bad[:, 64:] = sees[:, None]
+            assert torch.equal(torch.isnan(out[0, :, h]), bad), (window, h)
+        assert torch.isfinite(lse).all()
+
+
 # ---- refusals --------------------------------------------------------------------------------------------------
 def test_append_refuses_what_asks_for_a_gradient():
     cache = ra.KVCache4(1, 1, 64, 64)
