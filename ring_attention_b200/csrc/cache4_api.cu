@@ -86,8 +86,11 @@ int ra_cache4_evict(const ra_cache4_t* cache, int32_t keep, int32_t recent, cons
   if ((rc = check_cache(out, "out", &o))) return rc;
   if (o.b != c.b || o.hkv != c.hkv || o.d != c.d || o.cap < keep)
     return fail(-71, "out must have the cache's b, hkv and d and room for %d rows", keep);
-  if (o.k == c.k && (o.cap != c.cap || o.v != c.v || o.kl != c.kl || o.vl != c.vl || o.pos != c.pos || o.weight != c.weight ||
-                     o.len != c.len || o.seen != c.seen))
+  const void* from[] = {c.k, c.v, c.kl, c.vl, c.pos, c.weight, c.len, c.seen};
+  const void* to[] = {o.k, o.v, o.kl, o.vl, o.pos, o.weight, o.len, o.seen};
+  int shared = 0;
+  for (int i = 0; i < 8; ++i) shared += from[i] == to[i];
+  if (shared && (shared < 8 || o.cap != c.cap))
     return fail(-72, "out must be the cache itself or share nothing with it");
   if (recent < 0 || recent > keep) return fail(-73, "recent must be between 0 and keep (got %d)", recent);
   if (!workspace || workspace_bytes < need) return fail(-74, "evict needs a workspace of %lld bytes", (long long)need);

@@ -6,7 +6,8 @@ import subprocess
 import numpy as np
 import pytest
 
-from tests.test_cache4_host import ROOT
+from ring_attention_b200._lib import lib
+from tests.test_cache4_host import ROOT, _cache
 
 
 @pytest.fixture(scope="module")
@@ -26,3 +27,17 @@ def test_parts_are_read_within_the_workspace_whatever_an_item_s_note_holds(shim)
         for first in words:
             for last in words:
                 assert bool(shim.ra_host_cache_note_holds(first, last, ctas)) == (0 <= first <= last < ctas)
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_limits", "v_limits", "positions", "weights", "lengths", "seen"])
+def test_an_eviction_into_a_cache_that_shares_an_array_is_refused(name):
+    """All arrays of `out` are the cache's own (in place, the same capacity), or none."""
+    names = ["k", "v", "k_limits", "v_limits", "positions", "weights", "lengths", "seen"]
+    other = {x: 0x100000 + 0x1000 * i for i, x in enumerate(names)}
+    assert all(v != getattr(_cache(), x) for x, v in other.items())
+    one = C.c_void_p(0x1000)
+    shares_one = {**other, name: getattr(_cache(), name)}
+    all_but_one = {name: other[name]}
+    for arrays in (shares_one, all_but_one):
+        assert lib.ra_cache4_evict(C.byref(_cache()), 8, 0, C.byref(_cache(**arrays)), one, 1 << 40, None) == -72
+    assert lib.ra_cache4_evict(C.byref(_cache()), 8, 0, C.byref(_cache(capacity=192)), one, 1 << 40, None) == -72
