@@ -242,5 +242,7 @@ def cache_attention(
                                           scale, C.byref(mod) if mod is not None else None, _ptr(weights_out), _ptr(ws), nbytes,
                                           stream))
     elif weights_out is not None and weights_out.data_ptr() != cache.weights.data_ptr():
-        weights_out.copy_(cache.weights)
+        # (no query, no probability; slots behind the last row are left as they are, as in any call)
+        live = torch.arange(cache.capacity, device=cache.device) < cache.lengths[:, None, None]
+        weights_out.copy_(torch.where(live, cache.weights, weights_out))
     return (out, lse) if return_lse else out

@@ -211,6 +211,21 @@ def test_no_rows_at_start_drop_what_is_behind(dtype):
     assert cache.positions[:, 1, :].gather(1, cache.lengths[:, None].long() - 1).flatten().tolist() == [7, 0, 30]
 
 
+# ---- weights ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lq,room", [(0, None), (1, None), (70, ROOM)])
+def test_weights_of_slots_behind_the_last_row_are_left(lq, room):
+    f = Filled(41, [0, 5, 64, 100], 2, 64, BF16, capacity=room)
+    f.cache.weights.copy_(torch.rand_like(f.cache.weights))
+    w = torch.full_like(f.cache.weights, -3.0)
+    q = _rand(f.rng, (4, lq, 2, 64), BF16)
+    out = ra.cache_attention(q, f.cache, weights_out=w)
+    assert out.shape == q.shape
+    for i, n in enumerate(f.lengths):
+        assert (w[i, :, n:] == -3.0).all()
+        more = w[i, :, :n] - f.cache.weights[i, :, :n]
+        assert (more > 0).all() if lq else (more == 0).all()
+
+
 # ---- NaN under masks -------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,lq,room", [(F32, 2, None), (F32, 2, ROOM), (BF16, 2, None), (BF16, 2, ROOM), (BF16, 40, None), (BF16, 70, ROOM)])
 @pytest.mark.parametrize("at", [0, 130, 199])
