@@ -367,6 +367,8 @@ int ra_cache4_read(const ra_cache4_t* cache, const ra_tensor_t* k, const ra_tens
  * are the last lq tokens); its other fields are not read.
  * weights_out (may be NULL) float32 [b, hkv, capacity]: cache->weights plus, for each row, the sum of
  * its probabilities over the lq queries and the heads that share it; it may be cache->weights itself.
+ * (Probabilities of this call: over a part of a cache held apart they add up to 1 over the part.  The parts' results are
+ * joined by lse; one that sees no row, NaN and -inf, is left out.)
  * Slots behind the last row are left as they are.  Results are the same bits at every call.
  * Channels of q are below 2^100 in magnitude (beyond, scores may leave the range of float32 on the way), and so are those of
  * the values (beyond, a key whose probability is 2^-20 or less of such a row's may be missing from the sum).

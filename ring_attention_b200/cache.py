@@ -193,9 +193,11 @@ def cache_attention(
     `bias_fn`: None (every row is visible) or a `ScoreMod` (causal, window, ALiBi) over the rows' positions and
     `q_positions` [b, lq]; by default the queries are the last lq tokens given to the cache.  A query that sees
     no row gets NaN and a log-sum-exp of -inf.  `return_lse`: also L [b, heads, lq] in float32, with which parts
-    of a cache held apart can be joined: out = sum exp(L_i - L) out_i.
+    of a cache held apart (the shards of a ring, say) can be joined: L = log sum exp(L_i), out = sum exp(L_i - L) out_i
+    over the parts with L_i > -inf; the others' out_i is NaN and is left out (a weight of 0 would not hide it).
     `weights_out` float32 [b, kv_heads, capacity]: receives `cache.weights` plus the probabilities of every row summed
-    over the queries and heads that read it; `cache.weights` itself accumulates in place.
+    over the queries and heads that read it; `cache.weights` itself accumulates in place.  The probabilities are those of
+    this call, over this cache: for a part held apart they add up to 1 over the part, not over the whole.
     There is no backward pass: the cache holds rounded copies."""
     if not isinstance(cache, KVCache4):
         raise TypeError("cache_attention reads a KVCache4")

@@ -211,6 +211,44 @@ def test_no_rows_at_start_drop_what_is_behind(dtype):
     assert cache.positions[:, 1, :].gather(1, cache.lengths[:, None].long() - 1).flatten().tolist() == [7, 0, 30]
 
 
+# ---- parts held apart ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,lq", [(F32, 1), (BF16, 1), (BF16, 70)])
+def test_parts_of_a_cache_held_apart_are_joined_by_their_log_sum_exps(dtype, lq):
+    """Four parts, as the ranks of a ring hold them; one is empty for the first sequence, others lie outside the window."""
+    rng = np.random.default_rng(51)
+    b, hkv, h, d, n, parts = 2, 2, 4, 128, 400, 4
+    k, v = _rand(rng, (b, n, hkv, d), dtype), _rand(rng, (b, n, hkv, d), dtype)
+    q = _rand(rng, (b, lq, h, d), dtype)
+    lengths, each = [290, 400], n // parts
+    q_pos = np.array([[x - lq + i for i in range(lq)] for x in lengths])
+    mod, window = ra.ScoreMod(causal=True, window=130), 130
+    outs, lses = [], []
+    for i in range(parts):
+        cache = ra.KVCache4(b, hkv, 64000, d)
+        at = slice(i * each, (i + 1) * each)
+        cache.append(k[:, at], v[:, at], counts=_i32([min(max(x - i * each, 0), each) for x in lengths]),
+                     positions=torch.arange(i * each, (i + 1) * each, device="cuda").expand(b, each).contiguous())
+        out, lse = ra.cache_attention(q, cache, q_positions=_i32(q_pos), bias_fn=mod, return_lse=True)
+        outs.append(out.double())
+        lses.append(lse.double())
+    assert torch.isneginf(lses[3][0]).all() and torch.isneginf(lses[0][0, :, -1]).all() and torch.isnan(outs[3][0]).all()
+    L = torch.logsumexp(torch.stack(lses), 0)
+    got = torch.zeros_like(outs[0])
+    for out, lse in zip(outs, lses):
+        share = torch.exp(lse - L).transpose(1, 2)[..., None]
+        got += torch.where(share > 0, share * out, torch.zeros_like(out))
+    # each part is off by what a call is: (2 es + 2^-20) 2 max |v|, and in bf16 by half a step of its own result and by the
+    # roundings of p and of values or p step code, together 2^-8, 2^-10 and 2^-11 * 15 / 8 of the largest value at most
+    kk, vv = O.values(_np(k)), O.values(_np(v))
+    for i, x in enumerate(lengths):
+        want = O.attend(_np(q)[i], kk[i, :x], vv[i, :x], np.tile(np.arange(x), (hkv, 1)), q_pos[i], d**-0.5, causal=True, window=window)
+        es = 64 * 2.0**-24 * want["size"] + 4 * 2.0**-24 * want["top"]
+        vmax = np.abs(vv[i, :x]).max()
+        tol = (2 * es + 2.0**-20)[None, :, None] * 4 * vmax + (0 if dtype == F32 else (2.0**-8 + 2.0**-10 + 2.0**-10) * vmax)
+        assert (np.abs(_np(got)[i] - want["out"]) <= tol).all()
+        assert (np.abs(_np(L)[i] - want["lse"]) <= 2 * es[:, None] + 2.0**-20 + 2.0**-21 * np.abs(want["lse"])).all()
+
+
 # ---- weights ---------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("lq,room", [(0, None), (1, None), (70, ROOM)])
 def test_weights_of_slots_behind_the_last_row_are_left(lq, room):
