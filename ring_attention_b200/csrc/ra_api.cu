@@ -5,6 +5,7 @@
 #include <cstdio>
 #include <cstring>
 
+#include "cache4.cuh"
 #include "common.cuh"
 #include "host_util.h"
 #include "tc_common.cuh"
@@ -173,7 +174,8 @@ int ra_device_status(uint32_t* bits) {
   if (v && (e = cudaMemcpy(word, &zero, sizeof(zero), cudaMemcpyHostToDevice)) != cudaSuccess)
     return fail_cuda(e, "cudaMemcpy");
   if (bits) *bits = v;
-  if (v) return fail(RA_ERR_DEVICE_STATUS, "a bounded wait ran out inside a kernel (status bits 0x%x)", v);
+  if (v)
+    return fail(RA_ERR_DEVICE_STATUS, v == kStCacheFull ? "rows were appended beyond a cache's capacity (status bits 0x%x)" : "a bounded wait ran out inside a kernel (status bits 0x%x)", v);
   return 0;
 }
 

@@ -302,3 +302,16 @@ def test_append_refuses_what_asks_for_a_gradient():
         cache.append(y, y)
     cache.append(y.detach(), x)
     assert cache.lengths.tolist() == [4]
+
+
+def test_the_status_call_says_what_happened_to_a_full_cache():
+    """Bit 17 alone is about dropped rows, not about a wait."""
+    cache = ra.KVCache4(1, 1, 64, 64)
+    x = torch.ones(1, 40, 1, 64, device="cuda")
+    cache.append(x, x)
+    cache.append(x, x)
+    bits = C.c_uint32(0)
+    assert _lib.lib.ra_device_status(C.byref(bits)) == _lib.RA_ERR_DEVICE_STATUS and bits.value == 1 << 17
+    text = _lib.lib.ra_last_error_string().decode()
+    assert "capacity" in text and "wait" not in text
+    assert ra.device_status() == 0
