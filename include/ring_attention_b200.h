@@ -327,7 +327,8 @@ int ra_ring_last_push(ra_ring_t* ring, int32_t backward, double* bytes, float* p
  * has lengths and seen zeroed, the other arrays may hold anything.  The number of rows of a
  * sequence (lengths) and of the tokens it was ever given (seen) live on the device and are read
  * there, so calls captured into a graph stay right while the cache grows.  No call synchronises.
- * Rows of a sequence may lie in any order: every row carries its position.  Calls on one cache
+ * Rows of a sequence may lie in any order: every row carries its position; the positions of a
+ * sequence's rows and queries lie less than 2^31 apart.  Calls on one cache
  * are ordered by their stream; calls that overlap on the GPU must not both write it.
  */
 typedef struct ra_cache4 {

@@ -13,7 +13,7 @@
 // that the tensor cores would truncate are exact (QueryTile, whole_number_scale): results are off by 1e-7 of themselves.
 //
 // The decoding form reads its cache once and does little with it (8 query rows share 144 bytes a key at 128
-// channels), so what bounds it is the stream of the cache and, close behind, the integer work that turns codes
+// channels): beside the stream of the cache most instructions are the integer work that turns codes
 // into operands.  That is why the products are warp-level MMAs with the codes on the M side: fragments are made
 // in registers straight from the packed words, where a tensor-memory MMA would want the decoded tile written to
 // shared memory and read back (from 64 query rows on that pays: cache4_prompt.cu).
@@ -28,9 +28,10 @@
 //
 // Measured, bf16, 128 channels, one token of 4 query heads a key/value head: 8 x 32768 keys of 8 heads 71 us (302 MB,
 // 4.2 TB/s), 64 x 819 to 8192 keys 91 us (345 MB, 3.8 TB/s), one sequence of 131072 keys 42 us (151 MB, 3.6 TB/s), where
-// a copy runs at 6.5 TB/s; the join 6 us.  From 151 to 302 MB the time grows at 5.2 TB/s, with 11 warps an SM (168
-// registers) and most instructions the operands' integer work; some 13 us do not depend on the length: launch, cuts, first
-// copies, cold code and joining, so that over the 42 us call 48 % of issue slots are used.
+// a copy runs at 6.5 TB/s; the join 6 us.  What bounds it is latency at few warps: 168 registers leave 11 warps an SM, which use
+// 49 to 53 % of issue slots and 51 to 57 % of the integer pipe, and wait longest for results of fixed latency (1.1 cycles an
+// instruction) and for the pipe (0.7), less for memory (0.4 to 0.7).  From 151 to 302 MB the time grows at 5.2 TB/s; some 13 us do
+// not depend on the length: launch, cuts, first copies, cold code and joining.
 // 16 heads of 1024 keys take 7.4 us in a graph, of which the launch and the fetch of cold code are the most.
 #include <cooperative_groups.h>
 
@@ -932,8 +933,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const __gri
 // (a tile alone is loaded once); from kSplitFrom tiles on the warps of a CTA divide the tiles, each goes over all kGroup
 // units that the CTA holds, and their sums are added in the order of the warps.  The next units are on their way
 // meanwhile.  Under a mask, units that no row sees are found by their positions and not fetched.
-// It reads half the cache and forms 64 scores a key; the integer work on the codes bounds it: 8 x 32768 keys of 8 heads, 4
-// rows each, 51 us (168 MB).  Divided / not, us of the pass: 8 x 8 heads of 4096 keys, 16 rows (2 tiles) 16 / 19, 24
+// It reads half the cache and forms 64 scores a key; what bounds it is waiting for its own loads (5.4 cycles an instruction with 18
+// warps an SM; 45 % of issue slots are used): 8 x 32768 keys of 8 heads, 4 rows each, 51 us (168 MB).  Divided / not, us of the pass: 8 x 8 heads of 4096 keys, 16 rows (2 tiles) 16 / 19, 24
 // rows 18 / 26, 256 rows 116 / 200, 4 x 8 heads of 16384, d 64, 16 rows 22 / 20, 24 rows 25 / 27; 4 heads of 2048 keys, 256 rows 10 / 104 (a tile's loading is 2 us that nothing hides).
 constexpr int kSplitFrom = 3;
 template <int D>
@@ -1165,7 +1166,9 @@ int sm_count() {
 
 // When the matrix form (cache4_prompt.cu) is taken: from this many query rows of a key/value head on, if the caches' capacity
 // times the 16-row tiles is at least this many keys.  It reads the cache once for 128 rows and not once for 16, but its
-// CTAs take longer to start.  Graph replays, us, this form / that one:
+// CTAs take longer to start.  All rules here go by the capacity, since the lengths are on the device and a captured call has to
+// stay right while the cache grows; they were measured with full caches, and one that holds little of its capacity takes the
+// form of a full one.  Graph replays, us, this form / that one:
 //   8 x 8 heads, 4096 keys, d 128: 32 rows 34 / 49, 64 rows 52 / 50, 256 rows 183 / 90;  d 256: 32 rows 87 / 112, 64 rows
 //   172 / 116, 256 rows 601 / 218
 //   4 heads, 16384 keys, d 128: 32 rows 20 / 27, 64 rows 29 / 28;  d 256: 48 rows 44 / 42, 64 rows 52 / 43

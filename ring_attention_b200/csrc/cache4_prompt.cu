@@ -26,8 +26,8 @@
 //
 // What bounds it is the chain of a unit (scores, exponentials, P, its product) with 18 warps an SM to fill its waits, which
 // registers limit: 44 % of issue slots are used, and a warp waits longest for what it reads of tensor memory and for the
-// other roles.  Measured, 16 heads over 4, 128 channels, 448 tokens that end a cache of 8192, causal: 88 us (29 GFLOP, 330
-// TFLOP/s), and 13 for the join; 256 channels, 640 rows on 2 heads of 28838 keys, causal: 146 us, 514 in the other form.
+// other roles.  Measured, 16 heads over 4, 128 channels, 448 tokens that end a cache of 8192, causal: 89 us (29 GFLOP, 330
+// TFLOP/s), and 14 for the join; 256 channels, 640 rows on 2 heads of 28838 keys, causal: 146 us, 514 in the other form.
 // TMEM columns: S0 [0, 64), S1 [64, 128), O [128, 128 + D); P lies in the first half of its S.
 #include <cuda_fp16.h>
 

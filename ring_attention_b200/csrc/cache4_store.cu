@@ -260,8 +260,8 @@ __device__ __forceinline__ void append_counters(const AppendParams& p, int b, co
 
 // A block takes kRowTile tokens of a sequence.  An octet of lanes has one group of 64 channels of K and of V and walks
 // down the tokens: reads run along a token's heads, and the rows of a head that the block writes are neighbours in the
-// cache.  Issue slots bound it (78 % used; 160 instructions for a lane's 8 channels, loads and stores with them): 2 x 32768
-// tokens of 16 heads, 128 channels, bf16, 694 MB in 209 us, 3.3 TB/s, where 106 us would be a copy's; 304 us before the
+// cache.  Issue slots bound it (76 % used; 160 instructions for a lane's 8 channels, loads and stores with them): 2 x 32768
+// tokens of 16 heads, 128 channels, bf16, 694 MB in 210 us, 3.3 TB/s, where 106 us would be a copy's; 304 us before the
 // bf16 form above of deciding levels.
 constexpr int kRowThreads = 256, kOctets = kRowThreads / 8, kRowTile = 16;
 struct OctetWalk {
@@ -326,7 +326,7 @@ __global__ void cache_counters_kernel(AppendParams p) {
 
 // ---- read --------------------------------------------------------------------------------------------
 // The same walk the other way: value = min + code step, rounded once.  2 x 32768 tokens of 16 heads, 128 channels, to bf16:
-// 694 MB in 142 us, 4.9 TB/s.
+// 694 MB in 143 us, 4.9 TB/s; it waits longest for its loads (8.3 cycles an instruction; 55 % of issue slots are used).
 // Code j of a word as a float (2^23 + code is 0x4b000000 | code; a conversion instruction runs at an eighth of the rate).
 __device__ __forceinline__ float code_of(uint32_t w, int j) {
   return __uint_as_float(((w >> (4 * j)) & 15u) | 0x4b000000u) - 8388608.f;
