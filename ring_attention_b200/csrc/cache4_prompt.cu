@@ -3,11 +3,11 @@
 // every key) and goes to the tensor-memory MMAs.
 //
 // A CTA has 128 query rows and walks over units of 64 keys.  It decodes a unit's K and V once, into fp16 operands in
-// shared memory,   k' = step (code - 8) 2^-e   and   v' = (min + step code) 2^-f,
-// and then per unit:  S = Q K'^T + (group sums of q) (mid 2^-e)^T,  p = exp2(S 2^e factor + f - m),  O += P V'.
-// step has 8 significant bits and |code - 8| is at most 8, so k' is exact in fp16 where step 2^-e is 2^-17 or more (a group
-// whose step is less has one below 2^-26 of its row's largest value, or its row a power of two of its own: the loss is 2^-31
-// of that value at most); the other part of a key, its groups' mid = min + 8 step times the sums of q over the groups, is one
+// shared memory,   k' = step (code - 8) 2^(9 - e)   and   v' = (min + step code) 2^(15 - f),
+// and then per unit:  S = Q K'^T + (group sums of q) (mid 2^(9 - e))^T,  p = exp2(S 2^(e - 9) factor + f - m),  O += P V'.
+// step has 8 significant bits and |code - 8| is at most 8, so k' is exact in fp16 where step 2^(9 - e) is 2^-17 or more (a row
+// with a smaller one takes a power of two of its own, and what is smaller still, below 2^-25 of its row's largest value, loses
+// 2^-30 of that); the other part of a key, its groups' mid = min + 8 step times the sums of q over the groups, is one
 // more step of the product, of two-part factors (22 bits each).  Scores, and L with them, so have fp32 accuracy as in the
 // other form.  v' and P are rounded by 2^-11 of themselves, values below 2^-19 of their row's largest by 2^-29 of that.
 // e and f are powers of two that bring the rows into fp16's range: largest values below 2^9 for K, where the two-part mids
@@ -43,13 +43,13 @@ using namespace ptx;
 
 constexpr int kThreads = 288, kRows = kPromptRows, kKeys = kCacheUnit;
 constexpr float kLog2e = 1.4426950408889634f, kHeadroom = 6.f, kGrow = 8.f;
-// Exponents of rows: their largest value is below 2^(exponent + kTopK) or 2^(exponent + kTopV).
+// A row's largest value is below 2^exponent, and below 2^kTopK or 2^kTopV as an operand.
 constexpr int kTopK = 9, kTopV = 15;
 constexpr int kLeastExp = -64;  // of that value, and that of a row that is not there
 constexpr float kLeastStep = 0x1p-17f;  // of K, from which on its products with codes are exact
-// p 2^(f - m) of a unit whose f lies below this may be less than a float holds where larger values elsewhere set m, while p
-// itself still counts in the sum of probabilities, which is then formed without f.
-constexpr int kFarExp = -11 - kTopV;
+// p 2^(f - m) of a unit whose f lies below the first may be less than a float holds where larger values elsewhere set m, while p
+// itself still counts in the sum of probabilities, which is then formed without f; so it is where 2^-f is no normal float.
+constexpr int kFarExp = -11, kMostExp = 126;
 constexpr int kRoom = 2, kSpan = 10;  // a unit's exponents may lie this far below its common one, which starts kRoom above
 // The common exponent after a unit of largest exponent `most` that did not fit.
 __device__ __forceinline__ int next_common(int common, int most) {
@@ -140,8 +140,8 @@ __device__ __forceinline__ uint32_t two_parts(float x) {
 }
 
 // Exponent of a row of K or V whose largest value is x >= 0 (infinity, too: a sum of limits that is just beyond).
-__device__ __forceinline__ int row_exponent(float x, bool v) {
-  return max((int)(__float_as_uint(x) >> 23) - 126, kLeastExp) - (v ? kTopV : kTopK);
+__device__ __forceinline__ int row_exponent(float x) {
+  return max((int)(__float_as_uint(x) >> 23) - 126, kLeastExp);
 }
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -225,8 +225,8 @@ struct KeyRow {
       if (!there || !finite) step[i] = mn[i] = 0.f;  // (rows behind the last hold anything)
       if (step[i] > 0.f) least = fminf(least, step[i]);
     }
-    const int own = there ? row_exponent(most(), v) : kLeastExp - kTopV;
-    const bool fits = !there || (own <= common && own >= common - kSpan && (v || least * two_to(-common) >= kLeastStep));
+    const int own = there ? row_exponent(most()) : kLeastExp;
+    const bool fits = !there || (own <= common && own >= common - kSpan && (v || least * two_to(kTopK - common) >= kLeastStep));
     const int e = fits ? common : own;
     (v ? side.f : side.e)[row] = e;
     (v ? side.bad_v : side.bad_k)[row] = bad;
@@ -236,7 +236,7 @@ struct KeyRow {
       side.most[warp] = largest;
       side.odd[warp] = odd;
     }
-    const float scale = two_to(-e);
+    const float scale = two_to((v ? kTopV : kTopK) - e);
     __half2 st[NG], off[NG];
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
@@ -296,7 +296,7 @@ __device__ __noinline__ uint32_t scores_by_key(uint32_t taddr, const Side& side,
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int key = c + j;
-      float x = fmaf(__uint_as_float(r[j]), factor * two_to(side.e[key]), (float)side.f[key]);
+      float x = fmaf(__uint_as_float(r[j]), factor * two_to(side.e[key] - kTopK), (float)side.f[key]);
       bool vis = key < live;
       if constexpr (MASKED) {
         const int kpos = side.pos[key];
@@ -465,14 +465,14 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
         if (unit < 0) break;
         const int live = len - unit * kKeys, f_unit = side.f[0];
         const int4 odds = *reinterpret_cast<const int4*>(side.odd);
-        const bool odd = (odds.x | odds.y | odds.z | odds.w) != 0, apart = odd || f_unit < kFarExp;
+        const bool odd = (odds.x | odds.y | odds.z | odds.w) != 0, apart = odd || f_unit < kFarExp || f_unit > kMostExp;
         bool plain = !odd && live >= kKeys;
         if constexpr (MASKED) {
           const int lo = min(side.least_pos[0], side.least_pos[1]), hi = max(side.most_pos[0], side.most_pos[1]);
           plain = plain && !(a.p.kinds & RA_MOD_ALIBI) && (!(a.p.kinds & RA_MOD_CAUSAL) || hi <= q_least) &&
                   (!(a.p.kinds & RA_MOD_WINDOW) || (long long)q_most - lo < a.p.window);
         }
-        float scale = factor * two_to(side.e[0]), off = (float)f_unit;
+        float scale = factor * two_to(side.e[0] - kTopK), off = (float)f_unit;
         const uint32_t phase = unit_phase >> buf & 1;
         if (!(ok = WARP_WAIT(&sh.bars[S_FULL + buf], phase))) break;
         tc_fence_after();
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
           float x[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j)  // column j of a chunk of 8 is channel (j >> 1) + 4 (j & 1)
-            x[(j & 8) + ((j & 7) >> 1) + 4 * (j & 1)] = nan_groups >> (col / 64) & 1 ? NAN : __uint_as_float(o[j]);
+            x[(j & 8) + ((j & 7) >> 1) + 4 * (j & 1)] = nan_groups >> (col / 64) & 1 ? NAN : __uint_as_float(o[j]) * two_to(-kTopV);
           if (!row_live) continue;
           if (!whole) {
 #pragma unroll
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, kPromptPerSm<D>) cache_prompt_kernel
       if (unit >= 0) {
         raw.load(a, bh, unit, thread, MASKED);
         // the first unit's largest exponent is the one to go by
-        const int own = (thread & 63) < len - unit * kKeys ? row_exponent(raw.most(), thread >= 64) : kLeastExp - kTopV;
+        const int own = (thread & 63) < len - unit * kKeys ? row_exponent(raw.most()) : kLeastExp;
         const int largest = __reduce_max_sync(0xffffffffu, own);
         if (lane == 0) sh.first[warp - 4] = largest;
       }
